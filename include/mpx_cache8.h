@@ -54,6 +54,20 @@ int mpx_kv_append8(const void* k, const void* v, void* k_pool, void* v_pool, flo
                    int cache_dtype, int32_t* errors, void* stream);
 
 /*
+ * The same for pages that hold more than a sequence's end: every slot that the call
+ * does not write keeps its value, before and behind the written ones. Only a call that
+ * writes all slots of a page starts it anew; any other has scale = max(old scale, need),
+ * and where it grew all other slots' codes are brought to it (once each, to the nearest).
+ * A page that holds nothing yet has the scale 0.
+ */
+int mpx_kv_write8(const void* k, const void* v, void* k_pool, void* v_pool, float* k_scales,
+                  float* v_scales, const int32_t* block_tables, const int32_t* start_pos,
+                  const int32_t* n_tokens, const int64_t* k_strides, const int64_t* v_strides,
+                  int B, int T, int H, int D, int num_blocks, int block_size, int max_blocks,
+                  int dtype, int code, const void* cos_cache, const void* sin_cache, int n_pos,
+                  int cache_dtype, int32_t* errors, void* stream);
+
+/*
  * Values of cached tokens: k_out, v_out (B, T, H, D) of `dtype`, contiguous,
  * 16-byte aligned. Row t of sequence b is position start_pos[b] + t; rows t >=
  * n_tokens[b], and rows without a page in the table, are zeros.

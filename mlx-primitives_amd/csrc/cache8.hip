@@ -16,6 +16,7 @@ struct Append8Params {
   int32_t* err;
   int64_t ks[3], vs[3];  // source (batch, token, head) strides in elements
   int B, T, H, D, num_blocks, bs, max_blocks, n_pos, pages;
+  int keep;  // slots that the call does not write keep their values, behind it too
 };
 
 // A sequence's tokens that have a place: positions [lo, hi).
@@ -205,7 +206,8 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(Append8Params p) {
   }
   const int e = need_exp8<I8>(amax);
   const float need = pow2f(e);
-  const float now = s0 == 0 ? need : fmaxf(was, need);
+  const bool anew = s0 == 0 && (!p.keep || s1 == p.bs);
+  const float now = anew ? need : fmaxf(was, need);
   // (a scale kept from before need not be a power of two)
   const float inv = now == need ? pow2f(-e) : 1.0f / now;
   auto place = [&](unsigned char* at, u32x2 x, u32x2 y) __attribute__((always_inline)) {
@@ -226,10 +228,11 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(Append8Params p) {
                                     x[4 * q + 3] * inv);
     place(dst + s * row, (u32x2){w[0], w[1]}, (u32x2){w[2], w[3]});
   });
-  if (s0 > 0 && now != was) {
+  const int rest = p.keep ? p.bs : s0;  // slots whose codes are brought to a larger scale
+  if (!anew && now != was) {
     const float f = was * inv;
-    for (int s = lane / LPR; s < s0; s += TPW) {
-      if (!on) continue;
+    for (int s = lane / LPR; s < rest; s += TPW) {
+      if (!on || (s >= s0 && s < s1)) continue;
       unsigned char* at = dst + s * row;
       u32x2 x = *(const u32x2*)(at + d0), y = *(const u32x2*)(at + d1);
 #pragma unroll
@@ -361,15 +364,15 @@ int check_cache8(const char* fn, int B, int T, int H, int D, int num_blocks, int
 
 using namespace mpx;
 
-extern "C" int mpx_kv_append8(const void* k, const void* v, void* k_pool, void* v_pool,
-                              float* k_scales, float* v_scales, const int32_t* block_tables,
-                              const int32_t* start_pos, const int32_t* n_tokens,
-                              const int64_t* k_strides, const int64_t* v_strides, int B, int T,
-                              int H, int D, int num_blocks, int block_size, int max_blocks,
-                              int dtype, int code, const void* cos_cache, const void* sin_cache,
-                              int n_pos, int cache_dtype, int32_t* errors, void* stream) {
+namespace {
+
+int append8(const char* fn, int keep, const void* k, const void* v, void* k_pool, void* v_pool,
+            float* k_scales, float* v_scales, const int32_t* block_tables,
+            const int32_t* start_pos, const int32_t* n_tokens, const int64_t* k_strides,
+            const int64_t* v_strides, int B, int T, int H, int D, int num_blocks, int block_size,
+            int max_blocks, int dtype, int code, const void* cos_cache, const void* sin_cache,
+            int n_pos, int cache_dtype, int32_t* errors, void* stream) {
   clear_error();
-  const char* fn = "mpx_kv_append8";
   const int rc = check_cache8(fn, B, T, H, D, num_blocks, block_size, max_blocks, dtype, code);
   if (rc != MPX_OK) return rc;
   const bool rope = cos_cache || sin_cache;
@@ -397,7 +400,7 @@ extern "C" int mpx_kv_append8(const void* k, const void* v, void* k_pool, void* 
   p.kscale = k_scales; p.vscale = v_scales;
   p.bt = block_tables; p.start = start_pos; p.ntok = n_tokens; p.err = errors;
   p.B = B; p.T = T; p.H = H; p.D = D; p.num_blocks = num_blocks; p.bs = block_size;
-  p.max_blocks = max_blocks; p.n_pos = n_pos;
+  p.max_blocks = max_blocks; p.n_pos = n_pos; p.keep = keep;
   // T tokens touch at most this many pages, wherever they start
   p.pages = (int)(((int64_t)T + block_size - 2) / block_size + 1);
   MPX_CHECK_ARG(B < 65535 && p.pages <= 65535, "%s: too many tokens in one call", fn);
@@ -414,6 +417,32 @@ extern "C" int mpx_kv_append8(const void* k, const void* v, void* k_pool, void* 
   }
   MPX_CHECK_HIP(hipGetLastError());
   return MPX_OK;
+}
+
+}  // namespace
+
+extern "C" int mpx_kv_append8(const void* k, const void* v, void* k_pool, void* v_pool,
+                              float* k_scales, float* v_scales, const int32_t* block_tables,
+                              const int32_t* start_pos, const int32_t* n_tokens,
+                              const int64_t* k_strides, const int64_t* v_strides, int B, int T,
+                              int H, int D, int num_blocks, int block_size, int max_blocks,
+                              int dtype, int code, const void* cos_cache, const void* sin_cache,
+                              int n_pos, int cache_dtype, int32_t* errors, void* stream) {
+  return append8("mpx_kv_append8", 0, k, v, k_pool, v_pool, k_scales, v_scales, block_tables,
+                 start_pos, n_tokens, k_strides, v_strides, B, T, H, D, num_blocks, block_size,
+                 max_blocks, dtype, code, cos_cache, sin_cache, n_pos, cache_dtype, errors, stream);
+}
+
+extern "C" int mpx_kv_write8(const void* k, const void* v, void* k_pool, void* v_pool,
+                             float* k_scales, float* v_scales, const int32_t* block_tables,
+                             const int32_t* start_pos, const int32_t* n_tokens,
+                             const int64_t* k_strides, const int64_t* v_strides, int B, int T,
+                             int H, int D, int num_blocks, int block_size, int max_blocks,
+                             int dtype, int code, const void* cos_cache, const void* sin_cache,
+                             int n_pos, int cache_dtype, int32_t* errors, void* stream) {
+  return append8("mpx_kv_write8", 1, k, v, k_pool, v_pool, k_scales, v_scales, block_tables,
+                 start_pos, n_tokens, k_strides, v_strides, B, T, H, D, num_blocks, block_size,
+                 max_blocks, dtype, code, cos_cache, sin_cache, n_pos, cache_dtype, errors, stream);
 }
 
 extern "C" int mpx_kv_load8(const void* k_pool, const void* v_pool, const float* k_scales,

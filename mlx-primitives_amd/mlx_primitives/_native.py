@@ -209,6 +209,8 @@ def load() -> ctypes.CDLL:
         lib.mpx_kv_append8.restype = ci
         lib.mpx_kv_append8.argtypes = [vp] * 9 + [_i64p] * 2 + [ci] * 9 + [vp] * 2 + [ci] * 2 + [
             vp] * 2
+        lib.mpx_kv_write8.restype = ci
+        lib.mpx_kv_write8.argtypes = lib.mpx_kv_append8.argtypes
         lib.mpx_kv_load8.restype = ci
         lib.mpx_kv_load8.argtypes = [vp] * 9 + [ci] * 9 + [vp]
         lib.mpx_paged_attend8.restype = ci
@@ -764,20 +766,22 @@ def qk_norm_rope_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
 def kv_append8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                k_scales: torch.Tensor, v_scales: torch.Tensor, block_tables: torch.Tensor,
                start_pos: torch.Tensor, n_tokens: torch.Tensor, errors: torch.Tensor,
-               rope: Optional[tuple]) -> None:
-    """Enqueue mpx_kv_append8 on the current stream: k, v (B, T, H, D)."""
+               rope: Optional[tuple], keep_rest: bool = False) -> None:
+    """Enqueue mpx_kv_append8, or mpx_kv_write8 (keep_rest: slots that are not written keep
+    their values), on the current stream: k, v (B, T, H, D)."""
     lib = load()
+    name = "mpx_kv_write8" if keep_rest else "mpx_kv_append8"
     B, T, H, D = k.shape
     cos, sin = rope if rope is not None else (None, None)
     with on_device(k.device):
-        rc = lib.mpx_kv_append8(
+        rc = getattr(lib, name)(
             k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scales.data_ptr(),
             v_scales.data_ptr(), block_tables.data_ptr(), start_pos.data_ptr(), n_tokens.data_ptr(),
             _bsh(k), _bsh(v), B, T, H, D, k_pool.shape[0], k_pool.shape[1], block_tables.shape[1],
             dtype_code(k.dtype), CODE8_FORMATS[k_pool.dtype], _ptr(cos), _ptr(sin),
             0 if cos is None else cos.shape[0], 0 if cos is None else dtype_code(cos.dtype),
             errors.data_ptr(), _stream_ptr(k.device))
-    _check(rc, "mpx_kv_append8 failed")
+    _check(rc, f"{name} failed")
 
 
 def kv_load8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor,

@@ -89,9 +89,8 @@ class BlockAllocator:
         self._v_pool = torch.zeros(shape, dtype=config.dtype, device=self._device)
         self._scales: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
         if config.is_8bit:
-            self._scales = tuple(
-                torch.zeros((num_blocks, config.num_heads), device=self._device)
-                for _ in range(2))
+            self._both_scales = torch.zeros((2, num_blocks, config.num_heads), device=self._device)
+            self._scales = (self._both_scales[0], self._both_scales[1])
         # Stack of free ids, lowest on top at start.
         self._free: List[int] = list(range(num_blocks - 1, -1, -1))
         self._ref_counts: List[int] = [0] * num_blocks
@@ -128,17 +127,32 @@ class BlockAllocator:
 
     def allocate(self, count: int = 1) -> List[int]:
         """Take `count` blocks (reference count 1 each); RuntimeError if the pool
-        has fewer free blocks (block_allocator.py:142-167)."""
+        has fewer free blocks (block_allocator.py:142-167). Blocks of 8 bits start
+        with the scale 0: what an earlier owner left in them stands for nothing."""
         with self._lock:
-            if count > len(self._free):
-                raise RuntimeError(
-                    f"Cannot allocate {count} blocks, only {len(self._free)} available")
-            out = []
-            for _ in range(count):
-                block_id = self._free.pop()
-                self._ref_counts[block_id] = 1
-                out.append(block_id)
+            out = self._take(count)
+            if self._scales is not None and out:
+                self._clear_scales(out)
             return out
+
+    def _take(self, count: int) -> List[int]:
+        if count > len(self._free):
+            raise RuntimeError(
+                f"Cannot allocate {count} blocks, only {len(self._free)} available")
+        out = []
+        for _ in range(count):
+            block_id = self._free.pop()
+            self._ref_counts[block_id] = 1
+            out.append(block_id)
+        return out
+
+    def _clear_scales(self, block_ids: List[int]) -> None:
+        first = min(block_ids)
+        if max(block_ids) - first + 1 == len(block_ids):
+            self._both_scales[:, first:first + len(block_ids)].zero_()
+        else:
+            ids = torch.tensor(block_ids).to(self._device)
+            self._both_scales.index_fill_(1, ids, 0.0)
 
     def _validate_block_id(self, block_id: int, context: str = "") -> None:
         if isinstance(block_id, bool) or not isinstance(block_id, int) or not (
@@ -180,7 +194,7 @@ class BlockAllocator:
             self._validate_block_id(block_id, "copy_on_write")
             if not self._enable_cow or self._ref_counts[block_id] <= 1:
                 return block_id
-            new_id = self.allocate(1)[0]
+            new_id = self._take(1)[0]
             self._k_pool[new_id].copy_(self._k_pool[block_id])
             self._v_pool[new_id].copy_(self._v_pool[block_id])
             for s in self._scales or ():
@@ -201,7 +215,9 @@ class BlockAllocator:
         block, through copy-on-write when the block is shared
         (block_allocator.py:299-331). Returns the id of the block written (the
         copy when one was made; the reference drops it, so a caller that keeps
-        a table must map the old id to this one)."""
+        a table must map the old id to this one). The other slots keep their
+        values (8-bit blocks: rounded once more where the write raises the
+        block's scale)."""
         with self._lock:
             self._validate_block_id(block_id, "set_block_data")
             target = self.copy_on_write(block_id) if self._enable_cow else block_id

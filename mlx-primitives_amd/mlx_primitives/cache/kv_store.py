@@ -138,6 +138,14 @@ def store_kv(
                 return words
             _raise_errors(words.tolist())
             return None
+    return _store(k_pool, v_pool, block_tables, k, v, start_positions, num_tokens, check, errors,
+                  rope, kv_scales)
+
+
+def _store(k_pool, v_pool, block_tables, k, v, start_positions, num_tokens=None, check=True,
+           errors=None, rope=None, kv_scales=None, keep_rest=False) -> Optional[torch.Tensor]:
+    """store_kv's general path; keep_rest (8-bit pools): slots that the call does not write
+    keep their values, also behind the last one written."""
     if k.ndim == 3:
         k, v = k[None], v[None]
         block_tables = block_tables.reshape(1, -1)
@@ -210,7 +218,7 @@ def store_kv(
         if k.numel() == 0:
             errors.zero_()  # (no kernel runs, which would write them)
         _native.kv_append8(k, v, k_pool, v_pool, *kv_scales, tables, starts, counts, errors,
-                           None if rope is None else (cos_cache, sin_cache))
+                           None if rope is None else (cos_cache, sin_cache), keep_rest)
     elif not _native.kv_append_clear(k, v, k_pool, v_pool, tables, starts, counts, errors,
                                    None if rope is None else (cos_cache, sin_cache)):
         errors.zero_()
@@ -286,8 +294,13 @@ def set_block_data(k_pool: torch.Tensor, v_pool: torch.Tensor, block_id: int, k:
     """Write k, v (length, heads, dim) into page block_id from slot start_pos.
 
     Same arguments and errors as BlockAllocator.set_block_data
-    (block_allocator.py:299-331, without the allocator's copy-on-write);
-    kv_scales as in store_kv.
+    (block_allocator.py:299-331, without the allocator's copy-on-write).
+
+    kv_scales as in store_kv, but that the slots which are not written keep their
+    values, before and behind the written ones: the page's scale stays or grows, and
+    where it grew their codes are rounded to it once. Writing all slots starts the page
+    anew. A page that holds nothing yet has to have the scale 0 (a new pool's, and what
+    BlockAllocator gives a block it hands out).
     """
     num_blocks, block_size = k_pool.shape[:2]
     if not 0 <= int(block_id) < num_blocks:
@@ -298,5 +311,5 @@ def set_block_data(k_pool: torch.Tensor, v_pool: torch.Tensor, block_id: int, k:
         raise ValueError(
             f"slots [{start_pos}, {start_pos + length}) do not fit a block of {block_size}")
     table = torch.full((1, 1), int(block_id), dtype=torch.int32, device=k_pool.device)
-    store_kv(k_pool, v_pool, table, k[:length][None], v[:length][None], start_pos, check=False,
-             kv_scales=kv_scales)
+    _store(k_pool, v_pool, table, k[:length][None], v[:length][None], start_pos, check=False,
+           kv_scales=kv_scales, keep_rest=kv_scales is not None)
