@@ -91,7 +91,10 @@ int mpx_kv_load8(const void* k_pool, const void* v_pool, const float* k_scales,
  *
  *   q, o       (B, Sq, H, D) of `dtype` through {batch, head, seq} strides, q
  *              16-byte aligned in base and strides; H a multiple of H_kv
- *   workspace  mpx_paged_attend8_workspace_bytes(...) bytes, 16-byte aligned
+ *   workspace  mpx_paged_attend8_call_workspace_bytes(...) bytes (positions: whether
+ *              query_start is given), 16-byte aligned; at most 256 MiB, whatever the
+ *              tables' width, or none. mpx_paged_attend8_workspace_bytes(...): enough for
+ *              any causal and query_start
  */
 int mpx_paged_attend8(const void* q, const void* k_pool, const void* v_pool,
                       const float* k_scales, const float* v_scales, const int32_t* block_tables,
@@ -102,6 +105,9 @@ int mpx_paged_attend8(const void* q, const void* k_pool, const void* v_pool,
                       int dtype, int code, void* workspace, size_t workspace_bytes, void* stream);
 size_t mpx_paged_attend8_workspace_bytes(int B, int Sq, int H, int H_kv, int D, int block_size,
                                          int max_blocks, int dtype);
+size_t mpx_paged_attend8_call_workspace_bytes(int B, int Sq, int H, int H_kv, int D,
+                                              int block_size, int max_blocks, int dtype,
+                                              int causal, int positions);
 
 #ifdef __cplusplus
 }

@@ -56,12 +56,14 @@ struct Attend8Params {
   int B, Sq, H, H_kv, G, D, num_blocks, bs, max_blocks, causal;
   int o_rows16;    // o's base and strides are multiples of 16 bytes
   int wave_heads;  // the waves of the register form take heads, not tokens
-  int part, max_parts, blocks, span;  // tokens a partition; row blocks and their rows
-  u32 magic;             // ceil(2^32 / bs): n / bs = n * magic / 2^32 for n * bs < 2^32
+  int part, max_parts;   // tokens of a partition, and how many there is room for
+  int reach, step;       // tokens that fit them; partitions of longer sequences grow, in
+                         // multiples of this power of two
+  int blocks, span;      // row blocks and their rows
+  u32 magic, shift;      // n / bs = n * magic / 2^(32 + shift) for n < 2^31
   float c;               // scale * log2(e)
 };
 
-constexpr int kMostPart8 = 65536;  // tokens of a partition (32-bit page look-ups)
 constexpr int kTile8 = 32;
 
 // Where a sequence's queries start: positions past any cache, or before all, are
@@ -77,6 +79,19 @@ __device__ __forceinline__ int seen8(const Attend8Params& p, int ctx, int b, int
 }
 __device__ __forceinline__ int context8(const Attend8Params& p, int b) {
   return max(0, min(p.cl[b], p.max_blocks * p.bs));
+}
+// Tokens of a partition of a sequence: the plan's where all of its tokens fit that many
+// partitions, else its tokens over the partitions. (The host knows the table's width, which
+// may be many times what is in it.)
+__device__ __forceinline__ int part8(const Attend8Params& p, int ctx, int b) {
+  const int seen = seen8(p, ctx, b, p.Sq * p.G - 1);
+  if (seen <= p.reach) return p.part;
+  const u32 n = (u32)p.max_parts, each = ((u32)seen + n - 1) / n;
+  return (int)((each + (u32)p.step - 1) & ~((u32)p.step - 1));
+}
+// Page of the n-th token of a table.
+__device__ __forceinline__ u32 page_of8(const Attend8Params& p, u32 n) {
+  return p.bs == 1 ? n : __umulhi(n, p.magic) >> p.shift;
 }
 
 template <int QT>
@@ -137,9 +152,11 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
   const int R = p.Sq * p.G, rho0 = blk * 16 * NR;
   const int ctx = context8(p, b);
   const int tmax = seen8(p, ctx, b, rho0 + 16 * NR - 1);
-  const int p0 = part * p.part, p1 = min(p0 + p.part, tmax);
-  if (p0 >= p1 && p.max_parts > 1) return;  // (the merge knows)
-  const int pg0 = p0 / p.bs, base = pg0 * p.bs;
+  const int tokens = part8(p, ctx, b);
+  const int p0 = part * tokens, p1 = min(p0 + tokens, tmax);
+  const bool alone = p.max_parts == 1 || tmax <= tokens;  // no other partition: o right away
+  if (p0 >= p1 && (!alone || part > 0)) return;  // (the merge knows)
+  const int pg0 = page_of8(p, p0), base = pg0 * p.bs;
   const int32_t* const table = p.bt + (int64_t)b * p.max_blocks + pg0;
 
   // The waves share the partition's tokens evenly, each a run [w0, w1). Its pages
@@ -162,7 +179,7 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
   };
   auto find = [&](int t0) __attribute__((always_inline)) {
     const u32 n = (u32)(min(t0 + kUnit * lane, edge) - base);
-    const u32 i = p.bs == 1 ? n : __umulhi(n, p.magic);
+    const u32 i = page_of8(p, n);
     return Found{table[i], n - i * (u32)p.bs};
   };
   auto open = [&](const Found& f) __attribute__((always_inline)) {
@@ -577,7 +594,7 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
     T* const row = (T*)p.o + b * p.os[0] + h * p.os[1] + sq * p.os[2];
     // VB dims from d on: o / l (no token: 0 / 0 = NaN), or a partition's sums.
     auto put = [&](int d, const float* x, float L) __attribute__((always_inline)) {
-      if (p.max_parts == 1) {
+      if (alone) {
         if (d >= p.D) return;
         float y[VB];
 #pragma unroll
@@ -590,7 +607,7 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
       }
     };
     auto put_ml = [&](float M, float L) __attribute__((always_inline)) {
-      if (p.max_parts > 1 && q4 == 0) {
+      if (!alone && q4 == 0) {
         p.ws_ml[2 * slot] = M;
         p.ws_ml[2 * slot + 1] = L;
       }
@@ -733,8 +750,10 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
   const int R = p.Sq * p.G, rho0 = blk * kRows8;
   const int ctx = context8(p, b);
   const int tmax = seen8(p, ctx, b, rho0 + kRows8 - 1);
-  const int p0 = part * p.part, p1 = min(p0 + p.part, tmax);
-  if (p0 >= p1 && p.max_parts > 1) return;  // (the merge knows)
+  const int tokens = part8(p, ctx, b);
+  const int p0 = part * tokens, p1 = min(p0 + tokens, tmax);
+  const bool alone = p.max_parts == 1 || tmax <= tokens;  // no other partition: o right away
+  if (p0 >= p1 && (!alone || part > 0)) return;  // (the merge knows)
 
   const int rho = rho0 + 32 * wave + i32;
   const bool have = rho < R;
@@ -770,11 +789,10 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
   const int n_tiles = p0 < p1 ? (p1 - p0 + BN - 1) / BN : 0;
 
   // The first wave's look-ups: lane = token of the tile.
-  const int pg0 = p0 / p.bs, base = pg0 * p.bs;
+  const int pg0 = page_of8(p, p0), base = pg0 * p.bs;
   const int32_t* const table = p.bt + (int64_t)b * p.max_blocks + pg0;
   auto page_of = [&](int t) __attribute__((always_inline)) {  // from the partition's first on
-    const u32 n = (u32)(t - base);
-    return p.bs == 1 ? n : __umulhi(n, p.magic);
+    return page_of8(p, (u32)(t - base));
   };
   auto page_id = [&](int it) __attribute__((always_inline)) {
     const int t = p0 + it * BN + lane;
@@ -1009,7 +1027,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
   }
 
   l = pair_sum32(l);
-  if (p.max_parts == 1 && p.o_rows16) {
+  if (alone && p.o_rows16) {
     // Rows leave through the wave's part of the idle tiles, 16 bytes a lane and whole
     // rows an instruction, instead of 8-byte pieces of 32 rows (its own LDS only:
     // nothing to wait for but its own writes).
@@ -1040,12 +1058,12 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
     return;
   }
   const int64_t part_slot = (((int64_t)b * p.H + h) * p.Sq + sq) * p.max_parts + part;
-  if (p.max_parts > 1 && have && h2 == 0) {
+  if (!alone && have && h2 == 0) {
     p.ws_ml[2 * part_slot] = m;
     p.ws_ml[2 * part_slot + 1] = l;
   }
   if constexpr (DK <= 128) {
-    if (p.max_parts > 1) {  // the same way for a partition's sums
+    if (!alone) {  // the same way for a partition's sums
       const float back = ref * (1.f / kUp);
       constexpr int SB = 4 * DK;  // bytes of a row of sums
       unsigned char* const own = &tile[0][0][0] + wave * 32 * SB;
@@ -1074,7 +1092,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
   }
   if (!have) return;
   // This lane's dims of its row: 32 d + 8 (e / 4) + 4 h2 + e % 4.
-  if (p.max_parts == 1) {
+  if (alone) {
     // (no token: 0 / 0 = NaN)
     const float inv = l == 0.f ? NAN : ref * (1.f / kUp) / l;
     T* out = (T*)p.o + b * p.os[0] + h * p.os[1] + sq * p.os[2];
@@ -1112,9 +1130,18 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
   const int64_t rows = (int64_t)p.B * p.H * p.Sq;
   const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
   if (row >= rows) return;
-  const int sq = (int)(row % p.Sq);
-  const int64_t bh = row / p.Sq;
-  const int h = (int)(bh % p.H), b = (int)(bh / p.H);
+  int sq, h, b;
+  if (rows < (1ll << 32)) {  // (a division of 64 bits takes some hundred instructions)
+    const u32 bh = (u32)row / (u32)p.Sq;
+    sq = (int)((u32)row - bh * (u32)p.Sq);
+    b = (int)(bh / (u32)p.H);
+    h = (int)(bh - (u32)b * (u32)p.H);
+  } else {
+    const int64_t bh = row / p.Sq;
+    sq = (int)(row - bh * p.Sq);
+    b = (int)(bh / p.H);
+    h = (int)(bh - (int64_t)b * p.H);
+  }
   const int rho = sq * p.G + h % p.G;
   const float* ml = p.ws_ml + 2 * row * p.max_parts;
   const float* wo = p.ws_o + row * p.max_parts * DK + 4 * lane;
@@ -1125,6 +1152,18 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
   // many were written) is known; what was not written is left out below.
   const int first = WAVES == 1 ? 0 : 8 * wave;
   int n = p.max_parts;
+  bool alone = false;  // one partition or no token: o is there
+  auto written = [&]() __attribute__((always_inline)) {
+    const int ctx = context8(p, b);
+    const int tmax = seen8(p, ctx, b, rho / p.span * p.span + p.span - 1);
+    const int tokens = part8(p, ctx, b);
+    alone = tmax <= tokens;
+    n = (tmax + tokens - 1) / tokens;
+  };
+  if (WAVES == 1 && rows > 16384) {  // (the loads themselves count there)
+    written();
+    if (alone) return;
+  }
   for (int i0 = first; i0 < n; i0 += 8 * WAVES) {
     const int have = min(8, p.max_parts - i0);
     float2 mli = make_float2(-INFINITY, 0.f);
@@ -1134,8 +1173,8 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
     for (int u = 0; u < 8; ++u)
       ov[u] = u < have && on ? *(const f32x4*)(wo + (int64_t)(i0 + u) * DK) : (f32x4){0.f, 0.f, 0.f, 0.f};
     if (i0 == first) {
-      const int tmax = seen8(p, context8(p, b), b, rho / p.span * p.span + p.span - 1);
-      n = (tmax + p.part - 1) / p.part;
+      written();
+      if (alone) break;
     }
     const int c = n - i0;
     const float mi = lane < min(c, 8) ? mli.x : -INFINITY, li = mli.y;
@@ -1156,14 +1195,16 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
       acc += wu * ov[u];
     }
   }
-  if constexpr (WAVES > 1) {
+  if constexpr (WAVES == 1) {
+    if (alone) return;
+  } else {
     if (lane == 0) {
       s_m[wave] = M;
       s_l[wave] = L;
     }
     if (wave > 0) *(f32x4*)s_acc[wave - 1][lane] = acc;
     __syncthreads();
-    if (wave > 0) return;
+    if (wave > 0 || alone) return;
     const float most = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
     const float keep = M == -INFINITY ? 0.f : fast_exp2(M - most);
     L *= keep;
@@ -1183,29 +1224,40 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
 
 namespace {
 
+// magic = ceil(2^(32 + shift) / bs) with the largest shift whose magic fits 32 bits: over by
+// less than bs <= 2^(shift + 1) in 2^(32 + shift), which n < 2^31 does not make a whole one of.
+// (A power of two divides exactly.)
+void page_magic8(int bs, u32& magic, u32& shift) {
+  shift = 0;
+  while ((2ll << shift) < bs) ++shift;
+  magic = (u32)(((1ull << (32 + shift)) + bs - 1) / bs);
+}
+
 int kernel_dim8(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 struct Plan8 {
-  int span, blocks, part, max_parts, wave_heads;
+  int span, blocks, part, max_parts, step, wave_heads;
 };
+
+constexpr int64_t kMostSums8 = 256ll << 20;  // bytes of partitions' sums of a call
 
 // Partitions of the rows form, from a model of its time in microseconds (fitted to
 // 100 measured pairs of shapes and partitions at head dim 128, which it meets within
 // 20%): a tile of 64 tokens takes a workgroup 1.65 alone on its CU and 2.45 with
 // another (512 workgroups are resident), 1.15 of a CU's time where the chip is full,
-// with half of the last partition behind (one a CU and twice the times at D 256); a start 4.5; the merge 4.5 more and each
-// partition's sums a write and a read at 5 TB/s. Sequences share no partition, so a
-// batch of prompts takes one each, 65 queries behind 4100 tokens (two sequences) ten of
-// 448: 37.7 us, against 42.4 with 16 of 256 and 43.5 with seven of 640.
-int rows_parts8(int64_t groups, int64_t rows, int64_t tokens, int DK) {
+// with half of the last partition behind (one a CU and twice the times at D 256); a start
+// 4.5; the merge 4.5 more and each partition's sums a write and a read at 5 TB/s. Sequences
+// share no partition, so a batch of prompts takes one each, 65 queries behind 4100 tokens
+// (two sequences) ten of 448: 37.7 us, against 42.4 with 16 of 256 and 43.5 with seven of 640.
+int64_t rows_parts8(int64_t groups, int64_t rows, int64_t tokens, int DK) {
   const double tile = DK / 128.0;
   const int64_t resident = DK <= 128 ? 512 : 256;
-  const int64_t least = (tokens + kMostPart8 - 1) / kMostPart8;
+  if (groups >= 2 * resident) return 1;  // (empty partitions would cost more than a tail)
   double best = 0.0;
   int64_t parts = 0;
-  for (int64_t n = least; n < least + 64; ++n) {
+  for (int64_t n = 1; n <= 64; ++n) {
     const int64_t tiles = (tokens + 64 * n - 1) / (64 * n);
-    if (n > least && tiles < 2) break;
+    if (n > 1 && tiles < 2) break;
     const int64_t wgs = groups * n;
     double t = tiles * tile * (wgs <= 256 || DK > 128 ? 1.65 : 2.45);
     if (wgs > resident)
@@ -1216,26 +1268,46 @@ int rows_parts8(int64_t groups, int64_t rows, int64_t tokens, int DK) {
       parts = n;
     }
   }
-  return (int)parts;
+  return parts;
 }
 
 // Rows of a block: 16 or 32 in the register form (16 for float32, whose operands
-// take the registers, and for head dims above 128), 128 above; and the tokens of
-// a partition.
-Plan8 plan8(int B, int Sq, int H, int H_kv, int D, int block_size, int max_blocks, int dtype) {
+// take the registers, and for head dims above 128), 128 above; and the partitions of the
+// tokens. Tokens are those that a row may see as far as the host knows: the table's width, or
+// for causal rows at positions of their own (from 0) the queries' number. The table may be far
+// wider than what is in it, so a plan is for both: as many partitions as the width asks for,
+// within kMostSums8, and as short as `near` tokens ask for; longer sequences spread over all of
+// them (part8). Two turns of 65 queries behind 4100 tokens: 38 us in tables of 4144 tokens, 39 in
+// tables of 32768 and of 131072 (138 and 169 with the partitions that 32768 and 131072 tokens
+// get); decode of 16 sequences of 301 to 4100: 23.6, 26.6, 26.6 (34 and 98).
+Plan8 plan8(int B, int Sq, int H, int H_kv, int D, int block_size, int max_blocks, int dtype,
+            bool causal, bool positions) {
   Plan8 s;
   const int64_t R = (int64_t)Sq * (H / H_kv);
   s.span = dtype == MPX_F32 || R <= 16 ? 16 : R <= 32 && D <= 128 ? 32 : kRows8;
   s.blocks = (int)((R + s.span - 1) / s.span);
-  const int64_t tokens = std::max<int64_t>(1, (int64_t)max_blocks * block_size);
+  int64_t width = std::max<int64_t>(1, (int64_t)max_blocks * block_size);
+  if (causal && !positions && Sq > 1) width = std::min<int64_t>(width, Sq);
   const int64_t groups = (int64_t)B * H_kv * s.blocks;
-  auto cut = [&](int64_t n, int64_t step) {  // n partitions or fewer, of whole steps
-    s.part = (int)std::min<int64_t>(((tokens + n - 1) / n + step - 1) / step * step, kMostPart8);
-    s.max_parts = (int)((tokens + s.part - 1) / s.part);
+  const int64_t room =
+      std::max<int64_t>(1, kMostSums8 / ((int64_t)B * H * Sq * (kernel_dim8(D) + 2) * 4));
+  // parts(tokens): how many partitions that many tokens ask for.
+  auto plan = [&](auto parts, int64_t near, int64_t step) {
+    const int64_t n = std::min(parts(width), room);
+    auto each = [&](int64_t tokens, int64_t k) {
+      return ((tokens + k - 1) / k + step - 1) / step * step;
+    };
+    int64_t part = each(width, n);
+    if (n > 1 && width > near + near / 4) part = std::min(part, each(near, parts(near)));
+    s.part = (int)part;
+    s.max_parts = (int)std::min(n, (width + part - 1) / part);
+    s.step = (int)step;
   };
   s.wave_heads = 0;
   if (s.span == kRows8) {
-    cut(rows_parts8(groups, (int64_t)B * H * Sq, tokens, kernel_dim8(D)), 64);
+    const int64_t rows = (int64_t)B * H * Sq;
+    plan([&](int64_t tokens) { return rows_parts8(groups, rows, tokens, kernel_dim8(D)); }, 4096,
+         64);
     return s;
   }
   // The waves of the register form take four heads of the same tokens, whose rows
@@ -1244,24 +1316,32 @@ Plan8 plan8(int B, int Sq, int H, int H_kv, int D, int block_size, int max_block
   // Only for few rows: the sums of a partition's rows go through memory. 64 decode
   // rows over 512 to 8192 tokens, 32 heads: 420 us, 433 with partitions of 1024 and
   // 428 of 256; with shares of one head 467 to 510.
-  const int64_t p512 = (tokens + 511) / 512;
+  // (A table may be wider than what is in it: 16384 of its tokens count. Eight sequences of 4096
+  // tokens, 32 heads over 8, in tables of 131072: 21 us, 33 with waves that take heads.)
+  const int64_t p512 = (std::min<int64_t>(width, 16384) + 511) / 512;
   if (R <= 32 && H_kv % 4 == 0 && groups / 4 * p512 >= 2048) {
     s.wave_heads = 1;
-    cut(std::min<int64_t>(p512, 64), 512);  // (a wide table costs no endless workspace)
+    plan([&](int64_t tokens) { return std::min<int64_t>((tokens + 511) / 512, 64); }, 2048, 512);
     return s;
   }
   // As many partitions as give each CU a workgroup, none above 1024 tokens where rows are
-  // few (contexts differ: the long ones have to spread; up to 64 partitions) or under 256 (128 of float32, whose products
-  // take longer); one where the table is no longer than 512 tokens of 16-bit queries.
+  // few (contexts differ: the long ones have to spread; up to 64 partitions) or under 256
+  // (128 of float32, whose products take longer); one where there are no more than 512 tokens
+  // for 16-bit queries.
   // 32 heads over 8 of D 128, bf16, us: one sequence of 512 tokens 8.3 (two
   // partitions 9.5), 8192 tokens 10.2 (of 1024: 13.5), 32768 19.6 (of 512: 21.5, of
   // 4096: 31.7); four of 8192 19.0 (of 512: 20.3); 40 of 586 to 8192 102 (of 2048:
   // 117, of 4096 123).
   const bool wide = dtype != MPX_F32;
   const int64_t least = wide ? 256 : 128;
-  int64_t n = std::min(std::max<int64_t>(1, 256 / groups), (tokens + least - 1) / least);
-  if (R <= 32) n = std::max(n, std::min<int64_t>((tokens + 1023) / 1024, 64));
-  cut(wide && tokens <= 512 ? 1 : n, 128);
+  plan([&](int64_t tokens) {
+    if (wide && tokens <= 512) return (int64_t)1;
+    int64_t n = std::min(std::max<int64_t>(1, 256 / groups), (tokens + least - 1) / least);
+    // (16 sequences of 301 to 4100 in tables of 131072: 26 us with room for 32, 33 for 64)
+    const int64_t most = std::min<int64_t>(64, std::max<int64_t>(32, 4096 / groups));
+    if (R <= 32) n = std::max(n, std::min((tokens + 1023) / 1024, most));
+    return n;
+  }, 2048, 128);
   return s;
 }
 
@@ -1323,12 +1403,26 @@ hipError_t launch_attend_code(const Attend8Params& p, int code, hipStream_t st) 
 
 using namespace mpx;
 
+extern "C" size_t mpx_paged_attend8_call_workspace_bytes(int B, int Sq, int H, int H_kv, int D,
+                                                         int block_size, int max_blocks, int dtype,
+                                                         int causal, int positions) {
+  if (B <= 0 || Sq <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || block_size <= 0 ||
+      max_blocks < 0)
+    return 0;
+  return ws_bytes8(B, Sq, H, D, plan8(B, Sq, H, H_kv, D, block_size, max_blocks, dtype,
+                                      causal != 0, positions != 0));
+}
+
 extern "C" size_t mpx_paged_attend8_workspace_bytes(int B, int Sq, int H, int H_kv, int D,
                                                     int block_size, int max_blocks, int dtype) {
   if (B <= 0 || Sq <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || block_size <= 0 ||
       max_blocks < 0)
     return 0;
-  return ws_bytes8(B, Sq, H, D, plan8(B, Sq, H, H_kv, D, block_size, max_blocks, dtype));
+  // (as much as any causal and query_start ask for)
+  return std::max(ws_bytes8(B, Sq, H, D, plan8(B, Sq, H, H_kv, D, block_size, max_blocks, dtype,
+                                               false, false)),
+                  mpx_paged_attend8_call_workspace_bytes(B, Sq, H, H_kv, D, block_size, max_blocks,
+                                                         dtype, 1, 0));
 }
 
 extern "C" int mpx_paged_attend8(const void* q, const void* k_pool, const void* v_pool,
@@ -1370,7 +1464,8 @@ extern "C" int mpx_paged_attend8(const void* q, const void* k_pool, const void* 
   MPX_CHECK_ARG((int64_t)Sq * H < (1LL << 30), "%s: too many queries in one call", fn);
   MPX_CHECK_ARG((int64_t)num_blocks * block_size < (1LL << 32) - 1, "%s: too many pages", fn);
   Attend8Params p;
-  const Plan8 s = plan8(B, Sq, H, H_kv, D, block_size, num_blocks ? max_blocks : 0, dtype);
+  const Plan8 s = plan8(B, Sq, H, H_kv, D, block_size, num_blocks ? max_blocks : 0, dtype,
+                        causal != 0, query_start != nullptr);
   const size_t need = ws_bytes8(B, Sq, H, D, s);
   MPX_CHECK_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0 &&
                               workspace_bytes >= need),
@@ -1390,8 +1485,9 @@ extern "C" int mpx_paged_attend8(const void* q, const void* k_pool, const void* 
   p.num_blocks = num_blocks; p.bs = block_size; p.max_blocks = num_blocks ? max_blocks : 0;
   // one query without a position of its own sees its whole context
   p.causal = causal && (query_start || Sq > 1);
-  p.part = s.part; p.max_parts = s.max_parts; p.blocks = s.blocks; p.span = s.span; p.wave_heads = s.wave_heads;
-  p.magic = (u32)(((1ull << 32) + block_size - 1) / block_size);
+  p.part = s.part; p.max_parts = s.max_parts; p.reach = s.part * s.max_parts; p.step = s.step;
+  p.blocks = s.blocks; p.span = s.span; p.wave_heads = s.wave_heads;
+  page_magic8(block_size, p.magic, p.shift);
   p.c = scale * kLog2e;
   p.ws_o = (float*)workspace;
   p.ws_ml = (float*)workspace + (size_t)B * H * Sq * s.max_parts * kernel_dim8(D);

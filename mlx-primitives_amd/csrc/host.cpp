@@ -52,7 +52,7 @@ namespace {
   X(mpx_kv_append8)                                                                         \
   X(mpx_kv_load8)                                                                           \
   X(mpx_paged_attend8)                                                                      \
-  X(mpx_paged_attend8_workspace_bytes)                                                      \
+  X(mpx_paged_attend8_call_workspace_bytes)                                                      \
   X(mpx_qk_norm_rope)                                                                       \
   X(mpx_qk_norm_rope_bwd)                                                                   \
   X(mpx_qk_norm_rope_bwd_workspace_bytes)                                                   \
@@ -582,8 +582,8 @@ PyObject* attend8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)c.D) : PyFloat_AsDouble(a[5]);
   const c10::DeviceGuard guard(dev);
   at::Tensor o = at::empty(q->sizes(), q->options()), ws;
-  const size_t need = api.mpx_paged_attend8_workspace_bytes((int)B, (int)Sq, (int)H, c.H, c.D, c.bs,
-                                                            c.mb, code);
+  const size_t need = api.mpx_paged_attend8_call_workspace_bytes(
+      (int)B, (int)Sq, (int)H, c.H, c.D, c.bs, c.mb, code, a[7] == Py_True, qs != nullptr);
   if (need) ws = bytes(need, *q);
   const int64_t qst[3] = {q->stride(0), q->stride(2), q->stride(1)};
   const int64_t ost[3] = {o.stride(0), o.stride(2), o.stride(1)};

@@ -218,6 +218,8 @@ def load() -> ctypes.CDLL:
             cf, ci, ci, ci, vp, ctypes.c_size_t, vp]
         lib.mpx_paged_attend8_workspace_bytes.restype = ctypes.c_size_t
         lib.mpx_paged_attend8_workspace_bytes.argtypes = [ci] * 8
+        lib.mpx_paged_attend8_call_workspace_bytes.restype = ctypes.c_size_t
+        lib.mpx_paged_attend8_call_workspace_bytes.argtypes = [ci] * 10
         global _host
         try:
             _host = _load_host(lib)
@@ -810,7 +812,8 @@ def paged_attend8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     nb, bs, H_kv = k_pool.shape[:3]
     width = block_tables.shape[1]
     code = dtype_code(q.dtype)
-    need = int(lib.mpx_paged_attend8_workspace_bytes(B, Sq, H, H_kv, D, bs, width, code))
+    need = int(lib.mpx_paged_attend8_call_workspace_bytes(
+        B, Sq, H, H_kv, D, bs, width, code, int(causal), int(query_start is not None)))
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     with on_device(q.device):
         rc = lib.mpx_paged_attend8(
