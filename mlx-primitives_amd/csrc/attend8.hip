@@ -147,8 +147,9 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
   const int i16 = lane & 15, q4 = lane >> 4;
   // The waves take four heads of the same tokens, or one head and a share each.
   const bool heads = p.wave_heads != 0;
-  const int hk = heads ? 4 * blockIdx.x + wave : blockIdx.x, b = blockIdx.z;
-  const int blk = blockIdx.y % p.blocks, part = blockIdx.y / p.blocks;
+  const int hs = heads ? p.H_kv >> 2 : p.H_kv;
+  const int blk = p.blocks == 1 ? 0 : (int)(blockIdx.x / (u32)hs), hx = blockIdx.x - blk * hs;
+  const int hk = heads ? 4 * hx + wave : hx, part = blockIdx.y, b = blockIdx.z;
   const int R = p.Sq * p.G, rho0 = blk * 16 * NR;
   const int ctx = context8(p, b);
   const int tmax = seen8(p, ctx, b, rho0 + 16 * NR - 1);
@@ -742,7 +743,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
   // ones, the shortest beside the longest (two prompts of 2048 tokens, 16 heads over
   // one: 62 us; 84 with one sequence after the other).
   u32 at = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-  const u32 wgs = gridDim.x * gridDim.y * gridDim.z, heads = gridDim.x * gridDim.y;
+  const u32 wgs = gridDim.x * gridDim.y * gridDim.z, heads = (u32)p.H_kv * (u32)p.B;
   if (DK <= 128 && wgs <= 512 && at >= 256) at = wgs - 1 - (at - 256);
   const int z = at / heads, head = at - z * heads;
   const int b = head / p.H_kv, hk = head - b * p.H_kv;
@@ -1345,6 +1346,14 @@ Plan8 plan8(int B, int Sq, int H, int H_kv, int D, int block_size, int max_block
   return s;
 }
 
+// Sizes that the grid has room for: 2^32 threads in x, 65535 workgroups in z.
+bool grid_fits8(int B, int Sq, int H, int H_kv, int dtype) {
+  const int64_t R = (int64_t)Sq * (H / H_kv);
+  const int64_t blocks = (R + 15) / 16;  // (those of the least rows)
+  return B <= 65535 && (dtype == MPX_F32 || R <= 32 ? blocks : (R + kRows8 - 1) / kRows8) * H_kv <
+                           (1 << 24);
+}
+
 size_t ws_bytes8(int B, int Sq, int H, int D, const Plan8& s) {
   if (s.max_parts == 1) return 0;
   return (size_t)B * H * Sq * s.max_parts * (kernel_dim8(D) + 2) * sizeof(float);
@@ -1361,8 +1370,7 @@ template <int QT, bool I8, int DK>
 void launch_attend_nr(const Attend8Params& p, dim3 grid, hipStream_t st) {
   if constexpr (QT != MPX_F32) {
     if (p.span == kRows8) {
-      hipLaunchKernelGGL((attend8_rows_kernel<QT == MPX_BF16, I8, DK>), dim3(p.H_kv, p.B, grid.y),
-                         dim3(256), 0, st, p);
+      hipLaunchKernelGGL((attend8_rows_kernel<QT == MPX_BF16, I8, DK>), grid, dim3(256), 0, st, p);
       return;
     }
     if constexpr (DK <= 128) {
@@ -1376,7 +1384,7 @@ void launch_attend_nr(const Attend8Params& p, dim3 grid, hipStream_t st) {
 }
 template <int QT, bool I8>
 hipError_t launch_attend(const Attend8Params& p, hipStream_t st) {
-  const dim3 grid(p.wave_heads ? p.H_kv / 4 : p.H_kv, p.blocks * p.max_parts, p.B);
+  const dim3 grid((p.wave_heads ? p.H_kv / 4 : p.H_kv) * p.blocks, p.max_parts, p.B);
   const int dk = kernel_dim8(p.D);
   if (dk == 64) launch_attend_nr<QT, I8, 64>(p, grid, st);
   else if (dk == 128) launch_attend_nr<QT, I8, 128>(p, grid, st);
@@ -1407,7 +1415,7 @@ extern "C" size_t mpx_paged_attend8_call_workspace_bytes(int B, int Sq, int H, i
                                                          int block_size, int max_blocks, int dtype,
                                                          int causal, int positions) {
   if (B <= 0 || Sq <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || block_size <= 0 ||
-      max_blocks < 0)
+      max_blocks < 0 || !grid_fits8(B, Sq, H, H_kv, dtype))
     return 0;
   return ws_bytes8(B, Sq, H, D, plan8(B, Sq, H, H_kv, D, block_size, max_blocks, dtype,
                                       causal != 0, positions != 0));
@@ -1416,7 +1424,7 @@ extern "C" size_t mpx_paged_attend8_call_workspace_bytes(int B, int Sq, int H, i
 extern "C" size_t mpx_paged_attend8_workspace_bytes(int B, int Sq, int H, int H_kv, int D,
                                                     int block_size, int max_blocks, int dtype) {
   if (B <= 0 || Sq <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || block_size <= 0 ||
-      max_blocks < 0)
+      max_blocks < 0 || !grid_fits8(B, Sq, H, H_kv, dtype))
     return 0;
   // (as much as any causal and query_start ask for)
   return std::max(ws_bytes8(B, Sq, H, D, plan8(B, Sq, H, H_kv, D, block_size, max_blocks, dtype,
@@ -1463,6 +1471,7 @@ extern "C" int mpx_paged_attend8(const void* q, const void* k_pool, const void* 
   MPX_CHECK_ARG((int64_t)H_kv * D < (1 << 24), "%s: head count too large", fn);
   MPX_CHECK_ARG((int64_t)Sq * H < (1LL << 30), "%s: too many queries in one call", fn);
   MPX_CHECK_ARG((int64_t)num_blocks * block_size < (1LL << 32) - 1, "%s: too many pages", fn);
+  MPX_CHECK_ARG(grid_fits8(B, Sq, H, H_kv, dtype), "%s: grid too large", fn);
   Attend8Params p;
   const Plan8 s = plan8(B, Sq, H, H_kv, D, block_size, num_blocks ? max_blocks : 0, dtype,
                         causal != 0, query_start != nullptr);
@@ -1471,7 +1480,6 @@ extern "C" int mpx_paged_attend8(const void* q, const void* k_pool, const void* 
                               workspace_bytes >= need),
                 "%s: 16-byte aligned workspace of %zu bytes required, %zu given", fn, need,
                 workspace_bytes);
-  MPX_CHECK_ARG((int64_t)s.blocks * s.max_parts <= 65535 && B <= 65535, "%s: grid too large", fn);
   p.q = q; p.kpool = (const unsigned char*)k_pool; p.vpool = (const unsigned char*)v_pool;
   p.kscale = k_scales; p.vscale = v_scales; p.bt = block_tables; p.cl = context_lens;
   p.qstart = query_start; p.slopes = alibi_slopes; p.o = o;

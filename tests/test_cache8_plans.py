@@ -58,3 +58,6 @@ def test_sizes_that_are_none(lib):
     call = lib.mpx_paged_attend8_call_workspace_bytes
     assert call(0, 1, 4, 4, 64, 16, 8, 2, 1, 0) == 0
     assert call(1, 1, 5, 4, 64, 16, 8, 2, 1, 0) == 0
+    # sizes that the launch refuses ask for nothing first
+    assert call(65536, 1, 4, 4, 64, 16, 1 << 16, 2, 1, 0) == 0
+    assert call(1, 1 << 26, 8, 1, 64, 16, 1 << 16, 0, 0, 0) == 0

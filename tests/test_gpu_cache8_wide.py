@@ -86,3 +86,37 @@ def test_partitions_of_more_than_65536_tokens(device, bs, Sq, H):
         off = 2 * ((D + 8) * 2.0 ** -24 * E + 2.0 ** -22 * (1 + E) + n * 2.0 ** -24) + 2.0 ** -8
         bound = off * size + 2.0 ** -8 * ref.abs() + n * 2.0 ** -24 * 4
         assert ((out[0, i].double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dt,Sq,G", [("f32", 131073, 8), ("bf16", 65536, 8), ("f16", 3, 7)])
+@pytest.mark.parametrize("behind", [False, True])
+def test_rows_in_any_number(device, dt, Sq, G, behind):
+    # More than 65535 blocks of 16 float32 rows; a table of 2^20 tokens. All rows against the
+    # formula in 64 bits, bounds as in check_attend (values of unit scale).
+    rng = np.random.default_rng(Sq)
+    n, D, bs = 75, 16, 16
+    tables, nb = spread_tables(rng, [n], bs)
+    tables = wide(tables, (1 << 20) // bs)
+    kp, vp, _ = random_cache(rng, nb, bs, 1, D, "e4m3", device)
+    scales = tuple(torch.full((nb, 1), 2.0 ** -8, device=device) for _ in range(2))
+    q = torch.randn((1, Sq, G, D), device=device,
+                    generator=torch.Generator(device=device).manual_seed(Sq)).to(DTYPES[dt])
+    first = 30 if behind else 0
+    out = paged_attention(q, kp, vp, torch.from_numpy(tables).to(device), i32([n], device),
+                          enable_gqa=True, kv_scales=scales,
+                          query_start=i32([first], device) if behind else None)
+    pages = torch.from_numpy(tables[0, :-(-n // bs)]).long().to(device)
+    k, v = (p[pages].flatten(0, 1)[:n, 0].double() * 2.0 ** -8 for p in
+            (kp.float(), vp.float()))
+    u = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dt]
+    for lo in range(0, Sq, 16384):
+        rows = q[0, lo:lo + 16384].double()
+        at = first + lo + torch.arange(len(rows), device=device)
+        x = (rows @ k.t() / 4).masked_fill(
+            torch.arange(n, device=device) > at[:, None, None], -math.inf)
+        w = torch.softmax(x, -1)
+        ref, size = w @ v, w @ v.abs()
+        E = (rows.abs() @ k.abs().t() / 4).amax(-1, keepdim=True)
+        off = 2 * ((D + 8) * 2.0 ** -24 * E + 2.0 ** -22 * (1 + E) + n * 2.0 ** -24)
+        bound = (off + u) * size + u * ref.abs() + n * 2.0 ** -38 * 448 * 2.0 ** -8 + 2.0 ** -24
+        assert ((out[0, lo:lo + 16384].double() - ref).abs() <= bound).all()
