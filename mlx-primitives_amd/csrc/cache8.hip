@@ -15,7 +15,7 @@ struct Append8Params {
   const int32_t *bt, *start, *ntok;
   int32_t* err;
   int64_t ks[3], vs[3];  // source (batch, token, head) strides in elements
-  int B, T, H, D, num_blocks, bs, max_blocks, n_pos, pages;
+  int B, T, H, D, num_blocks, bs, max_blocks, n_pos, pages, groups;
   int keep;  // slots that the call does not write keep their values, behind it too
 };
 
@@ -39,7 +39,7 @@ struct Span8 {
 __device__ void append8_errors(const Append8Params& p) {
   int neg = 0, past = 0, bad = 0, rope = 0;
   const int64_t cap = (int64_t)p.max_blocks * p.bs;
-  const u32 n = (u32)p.B * (u32)p.pages;  // (both under 65536)
+  const u32 n = (u32)p.B * (u32)p.pages;  // (under 2^31)
   for (u32 i0 = 0; i0 < n; i0 += 1024) {
     int page[4];
     bool look[4];
@@ -93,18 +93,24 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(Append8Params p) {
   typedef typename Elem<XT>::T T;
   typedef typename Elem<CT>::T C;
   constexpr int TPW = 64 / LPR;  // tokens at a time
-  if (blockIdx.z == gridDim.z - 1) {
-    if (blockIdx.x == 0 && blockIdx.y == 0) append8_errors(p);
+  const u32 index = blockIdx.y * gridDim.x + blockIdx.x;
+  if (index == 0) {
+    append8_errors(p);
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // workgroup 1 + (sequence * pages + page) * units' groups + group
+  const u32 wg = index - 1, seq_page = wg / (u32)p.groups;
+  if (seq_page >= (u32)p.B * (u32)p.pages) return;
+  const int b = p.pages == 1 ? (int)seq_page : (int)(seq_page / (u32)p.pages);
+  const int at_page = (int)(seq_page - (u32)b * (u32)p.pages);
+  const int unit = (int)(wg - seq_page * (u32)p.groups) * 4 +
+                   __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = unit >> 1;
   const bool isk = !(unit & 1);
   if (h >= p.H) return;
-  const int b = blockIdx.z;
   const Span8 seq(p, b);
-  const int64_t page_at = seq.first_page(p) + blockIdx.y;
+  const int64_t page_at = seq.first_page(p) + at_page;
   const int64_t base = page_at * p.bs;
   const int s0 = (int)max((int64_t)0, seq.lo - base), s1 = (int)min((int64_t)p.bs, seq.hi - base);
   if (s0 >= s1) return;
@@ -403,8 +409,12 @@ int append8(const char* fn, int keep, const void* k, const void* v, void* k_pool
   p.max_blocks = max_blocks; p.n_pos = n_pos; p.keep = keep;
   // T tokens touch at most this many pages, wherever they start
   p.pages = (int)(((int64_t)T + block_size - 2) / block_size + 1);
-  MPX_CHECK_ARG(B < 65535 && p.pages <= 65535, "%s: too many tokens in one call", fn);
-  const dim3 grid((2 * H + 3) / 4, p.pages, B + 1);
+  p.groups = (2 * H + 3) / 4;
+  const int64_t a_seq = (int64_t)p.pages * p.groups;
+  MPX_CHECK_ARG(B < 65535 && a_seq < (1ll << 31) && 1 + a_seq * B < (1ll << 31),
+                "%s: too many tokens in one call", fn);
+  const int64_t wgs = 1 + a_seq * B, wide = std::min<int64_t>(wgs, 1 << 20);
+  const dim3 grid((unsigned)wide, (unsigned)((wgs + wide - 1) / wide));
   hipStream_t st = (hipStream_t)stream;
   if (code == MPX8_INT8) {
     if (dtype == MPX_F32) launch_append8<MPX_F32, true>(p, cache_dtype, grid, st);

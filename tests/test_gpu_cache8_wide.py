@@ -1,6 +1,6 @@
-"""Attention over 8-bit pages in block tables that are far wider than what is in them (static
-tables of captured programs, ragged batches): the same answers as in narrow tables, for every
-form, and partitions of any length. Oracle and bounds are those of test_gpu_cache8.
+"""The 8-bit cache at the far ends of its sizes: attention in block tables that are far wider than
+what is in them (static tables of captured programs, ragged batches), partitions, rows and
+appends of any length. Oracle and bounds are those of test_gpu_cache8.
 """
 
 import math
@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from mlx_primitives.cache import paged_attention
+from mlx_primitives.cache import load_kv, paged_attention, store_kv
 from test_gpu_cache8 import CODES, DTYPES, check_attend, make, random_cache, spread_tables
 from test_gpu_cache8_paths import i32, wide
 
@@ -120,3 +120,35 @@ def test_rows_in_any_number(device, dt, Sq, G, behind):
         off = 2 * ((D + 8) * 2.0 ** -24 * E + 2.0 ** -22 * (1 + E) + n * 2.0 ** -24)
         bound = (off + u) * size + u * ref.abs() + n * 2.0 ** -38 * 448 * 2.0 ** -8 + 2.0 ** -24
         assert ((out[0, lo:lo + 16384].double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("bs,T", [(1, 70001), (16, 16 * 65600 + 5), (16, 1)])
+def test_appends_of_any_length(device, bs, T):
+    # More pages than 65535 in one call, and the pages of many sequences: what comes back is what
+    # went in, values that codes hold exactly.
+    H, D, B = 1, 16, 3
+    counts = [T, 1, max(1, T // 3)]
+    starts = [0, bs // 2, 3]
+    pages = [-(-(s + n) // bs) for s, n in zip(starts, counts)]
+    nb = sum(pages)
+    gen = torch.Generator(device=device).manual_seed(T)
+    perm = torch.randperm(nb, device=device, generator=gen).int()
+    tables = torch.full((B, max(pages)), -1, dtype=torch.int32, device=device)
+    at = 0
+    for b, n in enumerate(pages):
+        tables[b, :n] = perm[at:at + n]
+        at += n
+    k, v = (torch.randint(-8, 9, (B, T, H, D), device=device, generator=gen).float() for _ in "kv")
+    for x in (k, v):
+        x[..., 0] = 127.0  # (the scale of every page is 1)
+    kp = torch.zeros((nb, bs, H, D), dtype=torch.int8, device=device)
+    vp = torch.zeros_like(kp)
+    scales = tuple(torch.zeros((nb, H), device=device) for _ in range(2))
+    store_kv(kp, vp, tables, k, v, i32(starts, device), i32(counts, device), kv_scales=scales)
+    got = load_kv(kp, vp, tables, i32(starts, device), i32(counts, device), max_tokens=T,
+                  kv_scales=scales, dtype=torch.float32)
+    for x, y in zip(got, (k, v)):
+        for b, n in enumerate(counts):
+            assert torch.equal(x[b, :n], y[b, :n]) and not x[b, n:].any()
+    with pytest.raises(RuntimeError, match="Block index"):  # one token past the tables
+        store_kv(kp, vp, tables[:1], k[:1, -1:], v[:1, -1:], tables.shape[1] * bs, kv_scales=scales)
