@@ -411,6 +411,14 @@ bool tracked(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// Whether one is a dual tensor of forward-mode differentiation (which the general
+// path refuses).
+bool dual(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (t && t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 // A plain tensor on `dev`, or nullptr.
 const at::Tensor* plain_on(PyObject* o, c10::Device dev) {
   const at::Tensor* t = plain(o);
@@ -479,7 +487,7 @@ PyObject* store8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (code < 0 || dtype_code(*v) != code || k->dim() != 4 || v->sizes() != k->sizes() ||
       k->size(2) != c.H || k->size(3) != c.D || k->numel() == 0 ||
       !aligned_rows(*k, code == MPX_F32 ? 4 : 8) || !aligned_rows(*v, code == MPX_F32 ? 4 : 8) ||
-      c.bt->size(0) != k->size(0) || tracked({k, v}))
+      c.bt->size(0) != k->size(0) || tracked({k, v}) || dual({k, v, c.ks, c.vs}))
     Py_RETURN_NONE;
   const int64_t B = k->size(0), T = k->size(1);
   if (B >= 65535 || T >= INT32_MAX || !int32_vector(*start, B) || (count && !int32_vector(*count, B)))
@@ -489,7 +497,7 @@ PyObject* store8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!PyTuple_CheckExact(a[8]) || PyTuple_GET_SIZE(a[8]) != 2) Py_RETURN_NONE;
     cos = plain_on(PyTuple_GET_ITEM(a[8], 0), dev);
     sin = plain_on(PyTuple_GET_ITEM(a[8], 1), dev);
-    if (!table_pair(cos, sin, c.D)) Py_RETURN_NONE;
+    if (!table_pair(cos, sin, c.D) || dual({cos, sin})) Py_RETURN_NONE;
   }
   const int words = cos ? 4 : 3;
   if (err && (err->scalar_type() != at::kInt || err->numel() != words || !err->is_contiguous()))
@@ -531,7 +539,7 @@ PyObject* load8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t dt = PyLong_AsLongLong(a[7]);
   if (PyErr_Occurred()) return nullptr;
   if (!start || !count || T <= 0 || T >= INT32_MAX || B == 0 || c.H == 0 || dt < 0 || dt > 2 ||
-      !int32_vector(*start, B) || !int32_vector(*count, B))
+      !int32_vector(*start, B) || !int32_vector(*count, B) || dual({c.ks, c.vs}))
     Py_RETURN_NONE;
   const c10::DeviceGuard guard(dev);
   const auto opts = c.ks->options().dtype(dt == MPX_F32   ? at::kFloat
@@ -571,7 +579,8 @@ PyObject* attend8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int code = dtype_code(*q);
   if (code < 0 || q->dim() != 4 || q->size(3) != c.D || q->numel() == 0 ||
-      !aligned_rows(*q, code == MPX_F32 ? 4 : 8) || tracked({q, sl, c.ks, c.vs}))
+      !aligned_rows(*q, code == MPX_F32 ? 4 : 8) || tracked({q, sl, c.ks, c.vs}) ||
+      dual({q, sl, c.ks, c.vs}))
     Py_RETURN_NONE;
   const int64_t B = q->size(0), Sq = q->size(1), H = q->size(2);
   if (B > 65535 || Sq * H >= (1 << 30) || c.H == 0 ||
@@ -735,7 +744,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       B * S * (q.size(2) + k.size(2)) >= INT32_MAX || !aligned_rows(q, vec) ||
       !aligned_rows(k, vec) || wq.dim() != 1 || wq.size(0) != D || wk.sizes() != wq.sizes() ||
       !wq.is_contiguous() || !wk.is_contiguous() || !aligned(wq) || !aligned(wk) ||
-      !table_pair(t[4], t[5], (int)D) || tracked({t[4], t[5]}) || !PyLong_CheckExact(a[6]) ||
+      !table_pair(t[4], t[5], (int)D) || tracked({t[4], t[5]}) ||
+      dual({t[0], t[1], t[2], t[3], t[4], t[5]}) || !PyLong_CheckExact(a[6]) ||
       !PyFloat_CheckExact(a[7]))
     Py_RETURN_NONE;
   NormCall c{q, k, wq, wk, *t[4], *t[5], {}, {}, PyLong_AsLongLong(a[6]), PyFloat_AsDouble(a[7])};

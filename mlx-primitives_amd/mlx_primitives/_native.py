@@ -22,6 +22,7 @@ import warnings
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 # MPX_ATTN_LIB selects another build of the library (e.g. a tuning variant).
 _LIB_PATH = os.environ.get("MPX_ATTN_LIB") or os.path.join(
@@ -303,6 +304,16 @@ def require_no_grad(*tensors: Optional[torch.Tensor]) -> None:
         raise NotImplementedError(
             "mlx_primitives (MI355X build) implements the forward pass only; call it under "
             "torch.no_grad() or torch.inference_mode(), or pass detached tensors")
+
+
+def require_no_tangent(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuse dual tensors of forward-mode differentiation, whose tangents the outputs
+    would silently lack."""
+    if forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("mlx_primitives (MI355X build) has no forward-mode derivatives; "
+                                  "pass tensors without tangents")
 
 
 def dtype_code(dtype: torch.dtype) -> int:

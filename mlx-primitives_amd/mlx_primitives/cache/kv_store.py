@@ -181,6 +181,7 @@ def _store(k_pool, v_pool, block_tables, k, v, start_positions, num_tokens=None,
     if kv_scales is not None:
         _native.require_device(k_pool, *kv_scales)
         _native.require_no_grad(k, v)
+        _native.require_no_tangent(k, v, *kv_scales, *(rope or ()))
     elif (dim * es) % 16:
         raise NotImplementedError(
             f"store_kv: head_dim * element size must be a multiple of 16 bytes (dim={dim})")
@@ -278,6 +279,7 @@ def load_kv(
     if max_tokens < 0:
         raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
     dev = _native.require_device(k_pool, v_pool, block_tables, *kv_scales)
+    _native.require_no_tangent(*kv_scales)
     batch = block_tables.shape[0]
     starts = _i32(start_positions, dev, batch, "start_positions")
     counts = _i32(num_tokens, dev, batch, "num_tokens")

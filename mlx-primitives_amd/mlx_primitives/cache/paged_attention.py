@@ -174,6 +174,7 @@ def _attend8(q, k_pool, v_pool, block_tables, context_lens, scale, causal, alibi
     _native.dtype_code(q.dtype)
     _native.require_device(q, k_pool, v_pool, block_tables, context_lens, *kv_scales)
     _native.require_no_grad(q, alibi_slopes, *kv_scales)
+    _native.require_no_tangent(q, alibi_slopes, *kv_scales)
     if alibi_slopes is not None:
         alibi_slopes = alibi_slopes.to(device=q.device, dtype=torch.float32).contiguous()
         if alibi_slopes.numel() != q.shape[2]:

@@ -95,8 +95,8 @@ def qk_norm_rope(
     None) is set.
 
     Returns new contiguous tensors. Differentiable in q, k and both weights
-    (the tables get no gradient); the weights' gradients are summed in float32
-    in a fixed order. A call that is captured into a HIP graph with gradients is
+    (the tables get no gradient, and there are no forward-mode derivatives); the
+    weights' gradients are summed in float32 in a fixed order. A call that is captured into a HIP graph with gradients is
     refused (RuntimeError) while an eager autograd graph of one of its leaves,
     made on the default stream, is alive.
     """
@@ -138,6 +138,7 @@ def qk_norm_rope(
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     dev = _native.require_device(q, k, q_weight, k_weight, cos_cache, sin_cache)
+    _native.require_no_tangent(q, k, q_weight, k_weight, cos_cache, sin_cache)
     if torch.is_grad_enabled() and (cos_cache.requires_grad or sin_cache.requires_grad):
         raise NotImplementedError("qk_norm_rope: the cos/sin tables get no gradient; pass "
                                   "detached tables")
