@@ -713,9 +713,14 @@ def qk_norm_rope_new(*args):
 
 def live_leaf(*tensors) -> bool:
     """Whether a graph is being captured and one of the tensors is a leaf of an eager
-    autograd graph that was made on the default stream and is still alive."""
+    autograd graph that was made on the default stream and is still alive. Without the
+    host extension, which can tell, every leaf counts as one."""
     with on_device(tensors[0].device):
-        return bool(host().live_leaf(*tensors))
+        found = host().live_leaf(*tensors)
+        if found is None:
+            found = (torch.cuda.is_current_stream_capturing()
+                     and any(t.requires_grad and t.is_leaf for t in tensors))
+        return found
 
 
 _same_device = contextlib.nullcontext()

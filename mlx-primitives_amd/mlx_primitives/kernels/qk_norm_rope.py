@@ -96,9 +96,10 @@ def qk_norm_rope(
 
     Returns new contiguous tensors. Differentiable in q, k and both weights
     (the tables get no gradient, and there are no forward-mode derivatives); the
-    weights' gradients are summed in float32 in a fixed order. A call that is captured into a HIP graph with gradients is
-    refused (RuntimeError) while an eager autograd graph of one of its leaves,
-    made on the default stream, is alive.
+    weights' gradients are summed in float32 in a fixed order. A call that is captured
+    into a HIP graph with gradients is refused (RuntimeError) while an eager autograd
+    graph of one of its leaves, made on the default stream, is alive, and for any leaf
+    where the host extension is not loaded, which could tell.
     """
     if positions is None or errors is not None or not check:
         # the ordinary call, checked and launched in native code
@@ -163,9 +164,10 @@ def qk_norm_rope(
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, q_weight, k_weight)):
         if _native.live_leaf(q, k, q_weight, k_weight):
             raise RuntimeError("qk_norm_rope: a graph is being captured while an eager autograd "
-                               "graph of the same leaf, made on the default stream, is alive; its "
-                               "gradient could not be captured. Delete that graph's outputs first, "
-                               "or make it on a side stream")
+                               "graph of the same leaf, made on the default stream, is alive (or, "
+                               "without the host extension, may be); its gradient could not be "
+                               "captured. Delete that graph's outputs first, or make it on a side "
+                               "stream")
         out = _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, offset, pos, float(eps),
                                   errors)
     else:
