@@ -48,8 +48,16 @@ EXTRA_FLAGS = {"fa_fwd.hip": _MAX_ILP + _VGPR_MFMA,
 ARCH = "gfx950"
 
 
+def rocm_home() -> str:
+    for cand in (os.environ.get("ROCM_HOME"), os.environ.get("ROCM_PATH")):
+        if cand and os.path.isdir(cand):
+            return cand
+    return "/opt/rocm"
+
+
 def hipcc() -> str:
-    for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
+    for cand in (os.environ.get("HIPCC"), os.path.join(rocm_home(), "bin", "hipcc"),
+                 "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if cand and os.path.exists(cand):
             return cand
     raise RuntimeError("hipcc not found (ROCm is required to build libmpx_attn.so)")
@@ -97,7 +105,7 @@ def host_command(out: str) -> list[str]:
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
              "-I" + INCLUDE, "-I" + sysconfig.get_paths()["include"]]
             + ["-isystem" + d for d in cpp_extension.include_paths()]
-            + ["-D__HIP_PLATFORM_AMD__", "-isystem/opt/rocm/include"]
+            + ["-D__HIP_PLATFORM_AMD__", "-isystem" + os.path.join(rocm_home(), "include")]
             + [os.path.join(CSRC, HOST_SOURCE), "-o", out, "-L" + torch_lib, "-ltorch_python",
                "-ltorch_cpu", "-lc10", "-lc10_hip"])
 
