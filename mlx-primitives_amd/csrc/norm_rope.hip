@@ -275,6 +275,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(NormParams p) {
           dw[K][8 + e] = fmaf(gr[8 + e] * r, b, dw[K][8 + e]);
           y1[e] = r * fmaf(-a, m, gr[e] * wv[K][e]);
           y2[e] = r * fmaf(-b, m, gr[8 + e] * wv[K][8 + e]);
+          y1[e] = t.in ? y1[e] : 0.f;  // (also where a weight is not finite)
+          y2[e] = t.in ? y2[e] : 0.f;
         }
         if (live) {
           Halves<T> y;
