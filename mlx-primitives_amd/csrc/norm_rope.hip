@@ -129,14 +129,16 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormParams p) {
   typedef typename Elem<XT>::T T;
   typedef typename Elem<CT>::T C;
   constexpr int RPW = 64 / LPR;
-  if (p.pos && blockIdx.x == gridDim.x - 1) {
+  const u32 wg = blockIdx.y * gridDim.x + blockIdx.x;
+  if (p.pos && wg == gridDim.x * gridDim.y - 1) {
     norm_error(p);
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tok = item / p.parts, part = item - tok * p.parts;
-  if (tok >= p.tokens) return;
+  const u32 item = wg * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u32 token = item / (u32)p.parts;
+  if (token >= (u32)p.tokens) return;
+  const int tok = (int)token, part = (int)(item - token * (u32)p.parts);
   const int grp = lane / LPR, d = (lane % LPR) * 8, half = p.D / 2;
   const bool on = d < half;
   const int nq = (p.H + RPW - 1) / RPW, n_it = nq + (p.H_kv + RPW - 1) / RPW;
@@ -364,9 +366,12 @@ hipError_t launch_one(const NormParams& p, bool bwd, hipStream_t st) {
   if (bwd)
     hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<XT, CT, LPR>), dim3(bwd_groups(waves)), dim3(256),
                        0, st, p);
-  else
-    hipLaunchKernelGGL((qk_norm_rope_kernel<XT, CT, LPR>), dim3((waves + 3) / 4 + (p.pos != nullptr)),
-                       dim3(256), 0, st, p);
+  else {
+    // (a grid has room for 2^32 threads in x)
+    const int64_t wgs = (waves + 3) / 4 + (p.pos != nullptr), wide = std::min<int64_t>(wgs, 1 << 20);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<XT, CT, LPR>),
+                       dim3((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), dim3(256), 0, st, p);
+  }
   return hipGetLastError();
 }
 template <int XT, int CT>
