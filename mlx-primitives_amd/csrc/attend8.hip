@@ -25,9 +25,10 @@
 // a zero byte above it the fp16 number (k + 128) 2^-24, a subnormal, which the matrix
 // instructions take exactly; 128 times the sum of the other operand is taken off
 // again, for S before the sum starts, for O at its end. K's scales multiply S
-// (float32); V's multiply P, over the largest of them so far, so that P stays in
-// range: P is rounded once (relative error 2^-11) and starts at 2^14, which leaves
-// 28 binary orders of page scales before it loses bits.
+// (float32); V's multiply P, in the exponent. A row has two running maxima: of a score,
+// x, for the sum of weights, and of x + log2 of V's scale for P and O, so that P, which is
+// rounded once to fp16 (relative error 2^-11), starts at 2^14 for the largest contribution
+// and keeps its bits down to 2^-28 of that, however far apart the scales of V are.
 //
 // Decode is memory bound where it fills the chip: 64 sequences of 512 to 8192 tokens,
 // 32 heads of D 128, int8: 422 us and 7.6 for the merge, 2.29 GB at 5.4 TB/s (a large copy
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
   constexpr int NK = WHOLE8 ? 1 : 2, NV = WHOLE8 ? 1 : 8;  // pages of a lane's K rows and V rows
   constexpr bool F32 = QT == MPX_F32, RAW = I8 && !F32;    // RAW: codes as fp16's subnormal bits
   typedef typename Elem<QT>::T T;
-  __shared__ float s_ml[4][NR][16][2];
+  __shared__ float s_ml[4][NR][16][3];
   __shared__ __align__(16) float s_o[4][NR][4][64][VB];
 
   const int lane = threadIdx.x & 63;
@@ -270,20 +271,20 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
   least = __builtin_amdgcn_readfirstlane(least);
 
   f32x4 o[NR][VB];
-  float m[NR], l[NR];
+  // Running maxima, whole numbers, of x and of x + log2 of V's scale; sums of 2^(x - m).
+  float m[NR], my[NR], l[NR];
   f32x4 pw[NR];  // RAW: what the 128 of every code adds to O, alike for all dims
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    m[n] = -INFINITY;
+    m[n] = my[n] = -INFINITY;
     l[n] = 0.f;
     pw[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < VB; ++v) o[n][v] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  // P is 2^kStart at the running maximum and V's largest scale; the maximum moves
-  // where a row's grows by more than kSlack, so that O is seldom rescaled.
-  constexpr float kStart = F32 ? 0.f : 14.f, kSlack = F32 ? 8.f : 1.5f;
-  float sref = 0.f;  // largest of V's scales so far
+  // P is 2^kStart at its running maximum, which moves where a row's grows by more than
+  // kSlack, so that O is seldom rescaled; that of the sum has float32's range (kFar).
+  constexpr float kStart = F32 ? 0.f : 14.f, kSlack = F32 ? 8.f : 1.5f, kFar = 64.f;
   const u32 row_bytes = (u32)p.H_kv * (u32)p.D;
   // This lane's bytes of a row: K chunks 16 (q + 4 j), V bytes VB i. (Lanes past the
   // head dim read others of the row, which Q's zeros and the stores leave out.)
@@ -410,22 +411,14 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
         }
       }
     }
-    // V's reference: the largest scale so far, at least 2^-100 (so that its inverse
-    // is finite).
-    float most = 0x1p-100f;
+    // V's scales as 2^(ve + vl), ve whole: exact sums with the maxima. (Scales under 2^-120
+    // count as that.)
+    float ve[NV], vl[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) most = fmaxf(most, r.vs[j]);
-    if (__any(most > sref)) {
-      most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(pair_max32(most), sref);
-      const float f = sref / most;
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        pw[n] *= f;
-#pragma unroll
-        for (int v = 0; v < VB; ++v) o[n][v] *= f;
-      }
-      sref = most;
+    for (int j = 0; j < NV; ++j) {
+      const float v = fmaxf(r.vs[j], 0x1p-120f);
+      ve[j] = (float)__builtin_amdgcn_frexp_expf(v);
+      vl[j] = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(v));
     }
     float pv[NR][8];
 #pragma unroll
@@ -445,39 +438,49 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
         }
         k = 1.f;
       }
-      float mx = pv[n][0];
+      float mx = pv[n][0], ym = WHOLE8 ? 0.f : pv[n][0] + (ve[0] + vl[0]);
 #pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, pv[n][j]);
+      for (int j = 1; j < 8; ++j) {
+        mx = fmaxf(mx, pv[n][j]);
+        if constexpr (!WHOLE8) ym = fmaxf(ym, pv[n][j] + (ve[WHOLE8 ? 0 : j] + vl[WHOLE8 ? 0 : j]));
+      }
       mx *= k;
-      if (__any(mx > m[n] + kSlack)) {
+      if constexpr (WHOLE8) ym = mx + (ve[0] + vl[0]);
+      if (__any(ym > my[n] + kSlack || mx > m[n] + kFar)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        const float mn = fmaxf(m[n], pair_max32(mx));
-        const float alpha = m[n] == -INFINITY ? 0.f : fast_exp2(m[n] - mn);
-        l[n] *= alpha;
+        ym = fmaxf(ym, __shfl_xor(ym, 16, 64));
+        const float mn = fmaxf(m[n], ceilf(pair_max32(mx))), yn = fmaxf(my[n], ceilf(pair_max32(ym)));
+        const float alpha = my[n] == -INFINITY ? 0.f : fast_exp2(my[n] - yn);
+        l[n] *= m[n] == -INFINITY ? 0.f : fast_exp2(m[n] - mn);
         pw[n] *= alpha;
 #pragma unroll
         for (int v = 0; v < VB; ++v) o[n][v] *= alpha;
         m[n] = mn;
+        my[n] = yn;
       }
-      const float sub = m[n] == -INFINITY ? 0.f : m[n] - kStart;
+      const float ref = my[n] == -INFINITY ? 0.f : my[n] - kStart;
+      const float sub = m[n] == -INFINITY ? 0.f : m[n];
       if constexpr (WHOLE8) {
-        // The share of V's scale goes into the exponent (a page without one: 2^-60,
-        // nothing); the sum of the weights takes it out again.
-        const float share = fmaxf(r.vs[0] / sref, 0x1p-60f);
-        const float off = __builtin_amdgcn_logf(share) - sub;
+        // The sum of the weights takes V's scale out again. So that P is in float32's range for
+        // any weight that counts there, a scale counts as 2^-80 of the largest contribution's
+        // at least (nothing to O).
+        const float low = my[n] - m[n] - 80.f;  // (NaN before the first token)
+        const bool tiny = low > ve[0] + vl[0];
+        const float e = tiny ? low : ve[0], f = tiny ? 0.f : vl[0];
+        const float off = (e - ref) + f;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           pv[n][j] = fast_exp2(__builtin_fmaf(pv[n][j], k, off));
           sum += pv[n][j];
         }
-        l[n] = __builtin_fmaf(sum, 1.f / share, l[n]);
+        l[n] = __builtin_fmaf(sum, fast_exp2((ref - e - sub) - f), l[n]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float e = fast_exp2(__builtin_fmaf(pv[n][j], k, -sub));
-          l[n] += e;
-          pv[n][j] = e * (r.vs[WHOLE8 ? 0 : j] / sref);
+          const int at = WHOLE8 ? 0 : j;
+          l[n] += fast_exp2(pv[n][j] - sub);
+          pv[n][j] = fast_exp2(pv[n][j] + ((ve[at] - ref) + vl[at]));
         }
       }
     }
@@ -563,9 +566,13 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
     }
   }
 
-  // The waves meet once: each leaves its sums, in V's units, and takes a quarter
-  // of the dims of all four, over the largest maximum.
-  const float back = RAW ? sref * 0x1p24f : sref;
+  // The waves meet once: each leaves its sums and maxima and takes a quarter of the dims of
+  // all four. What leaves the workgroup is O over the sum of weights (no larger than V), and for
+  // a partition that sum with the maximum it stands over.
+  constexpr int kBack = RAW ? 24 : 0;  // (subnormal codes are 2^-24)
+  auto factor = [&](float y, float M) __attribute__((always_inline)) {  // 2^(y - kStart - M)
+    return y == -INFINITY ? 0.f : __builtin_amdgcn_ldexpf(1.f, (int)(y - M - kStart) + kBack);
+  };
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     l[n] += __shfl_xor(l[n], 16, 64);
@@ -573,6 +580,7 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
     if (!heads && q4 == 0) {
       s_ml[wave][n][i16][0] = m[n];
       s_ml[wave][n][i16][1] = l[n];
+      s_ml[wave][n][i16][2] = my[n];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -580,8 +588,7 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
       for (int v = 0; v < VB; v += 4) {
         f32x4 x;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          x[k] = o[n][v + k][e] = (o[n][v + k][e] - (RAW ? pw[n][0] : 0.f)) * back;
+        for (int k = 0; k < 4; ++k) x[k] = o[n][v + k][e] = o[n][v + k][e] - (RAW ? pw[n][0] : 0.f);
         if (!heads) *(f32x4*)&s_o[wave][n][e][lane][v] = x;
       }
   }
@@ -593,14 +600,15 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
     const int sq = rho / p.G, h = hk * p.G + rho - sq * p.G;
     const int64_t slot = (((int64_t)b * p.H + h) * p.Sq + sq) * p.max_parts + part;
     T* const row = (T*)p.o + b * p.os[0] + h * p.os[1] + sq * p.os[2];
-    // VB dims from d on: o / l (no token: 0 / 0 = NaN), or a partition's sums.
-    auto put = [&](int d, const float* x, float L) __attribute__((always_inline)) {
+    // 1 / l for a row's end (no token: 0 * inf = NaN), or a partition's.
+    auto over = [&](float L) __attribute__((always_inline)) {
+      return !alone && L == 0.f ? 0.f : 1.f / L;
+    };
+    // VB dims from d on.
+    auto put = [&](int d, const float* x) __attribute__((always_inline)) {
       if (alone) {
         if (d >= p.D) return;
-        float y[VB];
-#pragma unroll
-        for (int v = 0; v < VB; ++v) y[v] = x[v] / L;
-        store_row8<VB>(row + d, y, p.o_rows16);
+        store_row8<VB>(row + d, x, p.o_rows16);
       } else {
 #pragma unroll
         for (int v = 0; v < VB; v += 4)
@@ -614,12 +622,13 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
       }
     };
     if (heads) {
+      const float inv = over(l[n]), f = factor(my[n], m[n]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float x[VB];
 #pragma unroll
-        for (int v = 0; v < VB; ++v) x[v] = o[n][v][e];
-        put(4 * VB * q4 + VB * e, x, l[n]);
+        for (int v = 0; v < VB; ++v) x[v] = o[n][v][e] * inv * f;
+        put(4 * VB * q4 + VB * e, x);
       }
       put_ml(m[n], l[n]);
       continue;
@@ -633,12 +642,16 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float mw = s_ml[w][n][i16][0];
-      const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
-      L = fmaf(f, s_ml[w][n][i16][1], L);
-#pragma unroll
-      for (int v = 0; v < VB; ++v) acc[v] = fmaf(f, s_o[w][n][wave][lane][v], acc[v]);
+      L = fmaf(mw == -INFINITY ? 0.f : fast_exp2(mw - M), s_ml[w][n][i16][1], L);
     }
-    put(4 * VB * q4 + VB * wave, acc, L);
+    const float inv = over(L);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = factor(s_ml[w][n][i16][2], M);
+#pragma unroll
+      for (int v = 0; v < VB; ++v) acc[v] = fmaf(s_o[w][n][wave][lane][v] * inv, f, acc[v]);
+    }
+    put(4 * VB * q4 + VB * wave, acc);
     if (wave == 0) put_ml(M, L);
   }
 }
@@ -1064,8 +1077,8 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
     p.ws_ml[2 * part_slot + 1] = l;
   }
   if constexpr (DK <= 128) {
-    if (!alone) {  // the same way for a partition's sums
-      const float back = ref * (1.f / kUp);
+    if (!alone) {  // the same way for a partition's
+      const float back = l == 0.f ? 0.f : ref * (1.f / kUp) / l;
       constexpr int SB = 4 * DK;  // bytes of a row of sums
       unsigned char* const own = &tile[0][0][0] + wave * 32 * SB;
       static_assert(4 * 32 * SB <= sizeof(tile), "a wave's rows fit its part of the tiles");
@@ -1106,7 +1119,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
         if (at < p.D) store_row8<4>(out + at, y, p.o_rows16);
       }
   } else {
-    const float back = ref * (1.f / kUp);
+    const float back = l == 0.f ? 0.f : ref * (1.f / kUp) / l;
     float* out = p.ws_o + part_slot * DK + 4 * h2;
 #pragma unroll
     for (int d = 0; d < DK / 32; ++d)
@@ -1117,8 +1130,8 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
   }
 }
 
-// Joins the partitions of a row: weights 2^(m - M) over the largest maximum, then
-// o / l. A chain of latencies: 3.2 us for 128 rows of six partitions, 7.7 for 4160 of
+// Joins the partitions of a row, which are o / l each: weights l 2^(m - M) over the largest
+// maximum. A chain of latencies: 3.2 us for 128 rows of six partitions, 7.7 for 4160 of
 // ten (22 MB). WAVES (1 or 4) waves a row, which take eight partitions at a time in turn:
 // one round trip to memory joins 8 or 32.
 template <int QT, int WAVES>
@@ -1191,8 +1204,8 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       if (u >= c) break;
-      const float wu = __shfl(w, u, 64);
-      L = fmaf(wu, __shfl(li, u, 64), L);
+      const float wu = __shfl(w * li, u, 64);
+      L += wu;
       acc += wu * ov[u];
     }
   }

@@ -73,7 +73,9 @@ def paged_attention(
     (num_blocks, H_kv), for pools of 8-bit codes as store_kv writes them
     (torch.float8_e4m3fn or torch.int8), or any positive scales of the caller's; q is
     float32, float16 or bfloat16. Products of 16-bit queries are those of 16-bit
-    matrix instructions, sums and softmax float32. Slots that no sequence reaches
+    matrix instructions, sums and softmax float32. Scales of pages may be any factor
+    apart; only float16 queries of more than 32 rows a K/V head (16 above dim 128) want
+    K and V within float16's range. Slots that no sequence reaches
     may hold anything; a NaN among the values of a cached token (float8_e4m3fn only)
     may also reach queries up to 96 positions before it, whose causal weight of 0 it
     is multiplied with.
