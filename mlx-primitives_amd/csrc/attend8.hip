@@ -495,15 +495,25 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
             o[n][v] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pv[n][j], o[n][v], 0, 0, 0);
         }
     } else {
-      u32x4 pb[NR];
+      // (float16 outputs show P's rounding: what it leaves is a second operand)
+      constexpr int PP = QT == MPX_F16 ? 2 : 1;
+      u32x4 pb[PP][NR];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) pb[n][w] = pack2<false>(pv[n][2 * w], pv[n][2 * w + 1]);
+        for (int w = 0; w < 4; ++w) {
+          const u32 x = pack2<false>(pv[n][2 * w], pv[n][2 * w + 1]);
+          pb[0][n][w] = x;
+          if constexpr (PP == 2)
+            pb[PP - 1][n][w] = pack2<false>(pv[n][2 * w] - h2f<false>((uint16_t)x),
+                                            pv[n][2 * w + 1] - h2f<false>((uint16_t)(x >> 16)));
+        }
       if constexpr (RAW) {
         const u32x4 a = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};
 #pragma unroll
-        for (int n = 0; n < NR; ++n) pw[n] = mfma16x16x32<false>(a, pb[n], pw[n]);
+        for (int k = 0; k < PP; ++k)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) pw[n] = mfma16x16x32<false>(a, pb[k][n], pw[n]);
       }
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
@@ -531,7 +541,10 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
             a[k] = RAW ? bytes4(x[2 * k + 1], x[2 * k], 0x0c040c00u + 0x00010001u * e)
                        : decode2<false, false>(col[e][k >> 1], k & 1);
 #pragma unroll
-          for (int n = 0; n < NR; ++n) o[n][4 * w + e] = mfma16x16x32<false>(a, pb[n], o[n][4 * w + e]);
+          for (int k = 0; k < PP; ++k)
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+              o[n][4 * w + e] = mfma16x16x32<false>(a, pb[k][n], o[n][4 * w + e]);
         }
       }
     }
