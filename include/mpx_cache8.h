@@ -88,8 +88,8 @@ int mpx_kv_load8(const void* k_pool, const void* v_pool, const float* k_scales,
  * those of pages that no visible token is in; they and all slots that no sequence
  * reaches may hold anything. Scales may be any factor apart, but that float16 queries in more
  * than 32 rows (Sq H / H_kv; 16 above head dim 128) want K and V in float16's range: what is
- * under 2^-31 of a scale near it counts as nothing there. An e4m3 NaN in V may also reach rows that share a tile
- * with its token and do not see it (their weight of 0 times NaN).
+ * under 2^-31 of a scale near it counts as nothing there. An e4m3 NaN in V may also reach rows
+ * that share a tile with its token and do not see it (their weight of 0 times NaN).
  *
  *   q, o       (B, Sq, H, D) of `dtype` through {batch, head, seq} strides, q
  *              16-byte aligned in base and strides; H a multiple of H_kv

@@ -3,8 +3,9 @@
 //
 // The rows of one K/V head are its group's query heads for every query: row
 // rho = query * G + head of the group, in blocks of 16 NR rows. A workgroup
-// takes one block and one partition of the tokens; its four waves take tiles
-// of 32 tokens in turn and meet in LDS at the end; partitions meet in
+// takes one block and one partition of the tokens, of which each of its four waves
+// takes a quarter, one run, in tiles of 32; they meet in LDS at the end. Or its waves
+// take four heads and all of the partition each. Partitions meet in
 // attend8_merge_kernel.
 //
 // Codes go from memory to registers in the layout that the matrix
@@ -28,7 +29,8 @@
 // (float32); V's multiply P, in the exponent. A row has two running maxima: of a score,
 // x, for the sum of weights, and of x + log2 of V's scale for P and O, so that P, which is
 // rounded once to fp16 (relative error 2^-11), starts at 2^14 for the largest contribution
-// and keeps its bits down to 2^-28 of that, however far apart the scales of V are.
+// and keeps its bits down to 2^-28 of that, however far apart the scales of V are. bf16
+// outputs do not show that rounding; for fp16 ones what it leaves is a second operand.
 //
 // Decode is memory bound where it fills the chip: 64 sequences of 512 to 8192 tokens,
 // 32 heads of D 128, int8: 422 us and 7.6 for the merge, 2.29 GB at 5.4 TB/s (a large copy
@@ -449,7 +451,8 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
       if (__any(ym > my[n] + kSlack || mx > m[n] + kFar)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         ym = fmaxf(ym, __shfl_xor(ym, 16, 64));
-        const float mn = fmaxf(m[n], ceilf(pair_max32(mx))), yn = fmaxf(my[n], ceilf(pair_max32(ym)));
+        const float mn = fmaxf(m[n], ceilf(pair_max32(mx)));
+        const float yn = fmaxf(my[n], ceilf(pair_max32(ym)));
         const float alpha = my[n] == -INFINITY ? 0.f : fast_exp2(my[n] - yn);
         l[n] *= m[n] == -INFINITY ? 0.f : fast_exp2(m[n] - mn);
         pw[n] *= alpha;
@@ -692,7 +695,10 @@ __global__ __launch_bounds__(256) void attend8_kernel(Attend8Params p) {
 // Decoded values: bf16 holds value = code * scale exactly where the scale is a
 // power of two (any other: rounded once, 2^-8). fp16 holds code * scale / reference *
 // 2^7, the reference of K being the largest scale of the tile, that of V the
-// largest so far: exact down to 2^-22 of it.
+// largest so far: exact down to 2^-22 of it. The weights are rounded to the type of the
+// values that they are multiplied with, as the framework's other 16-bit attention does
+// (bf16: outputs 2.1e-3 from 64 bits, one rounding alone is 1.6e-3); their float32 sum is
+// of the rounded ones, so that what they have in common cancels.
 constexpr int kRows8 = 128;
 
 template <int DK>
@@ -856,7 +862,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void attend8_rows_kernel(At
       f.ks[lane] = ks;
       f.vs[lane] = vs;
     }
-    const bool pow2 = __all((__float_as_uint(ks) & 0x7fffffu) == 0 && (__float_as_uint(vs) & 0x7fffffu) == 0);
+    const bool pow2 = __all(((__float_as_uint(ks) | __float_as_uint(vs)) & 0x7fffffu) == 0);
     if (lane == 0) {
       f.pow2 = pow2;
       f.valid = valid;
@@ -1198,7 +1204,8 @@ __global__ __launch_bounds__(256) void attend8_merge_kernel(Attend8Params p, int
     f32x4 ov[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      ov[u] = u < have && on ? *(const f32x4*)(wo + (int64_t)(i0 + u) * DK) : (f32x4){0.f, 0.f, 0.f, 0.f};
+      ov[u] = u < have && on ? *(const f32x4*)(wo + (int64_t)(i0 + u) * DK)
+                             : (f32x4){0.f, 0.f, 0.f, 0.f};
     if (i0 == first) {
       written();
       if (alone) break;
@@ -1421,7 +1428,8 @@ hipError_t launch_attend(const Attend8Params& p, hipStream_t st) {
   // (four waves a row where the rows alone leave the chip idle: 17 partitions of 32 rows 10.2 us
   // instead of 12.4 in all; for 4160 rows of ten 40.7 instead of 37.7)
   if (p.max_parts > 8 && rows <= 1024)
-    hipLaunchKernelGGL((attend8_merge_kernel<QT, 4>), dim3((unsigned)rows), dim3(256), 0, st, p, dk);
+    hipLaunchKernelGGL((attend8_merge_kernel<QT, 4>), dim3((unsigned)rows), dim3(256), 0, st, p,
+                       dk);
   else
     hipLaunchKernelGGL((attend8_merge_kernel<QT, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
                        st, p, dk);

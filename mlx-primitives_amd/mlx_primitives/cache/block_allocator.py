@@ -128,7 +128,8 @@ class BlockAllocator:
     def allocate(self, count: int = 1) -> List[int]:
         """Take `count` blocks (reference count 1 each); RuntimeError if the pool
         has fewer free blocks (block_allocator.py:142-167). Blocks of 8 bits start
-        with the scale 0: what an earlier owner left in them stands for nothing."""
+        with the scale 0 (a small device operation): what an earlier owner left in
+        them stands for nothing."""
         with self._lock:
             out = self._take(count)
             if self._scales is not None and out:

@@ -30,7 +30,8 @@ class _QkNormRopeFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, offset, positions, eps, errors):
-        q, k, q_weight, k_weight = _rows(q), _rows(k), _native.contiguous16(q_weight), _native.contiguous16(k_weight)
+        q, k = _rows(q), _rows(k)
+        q_weight, k_weight = map(_native.contiguous16, (q_weight, k_weight))
         out = _forward(q, k, q_weight, k_weight, cos, sin, offset, positions, eps, errors)
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.cfg = (offset, eps)
@@ -171,8 +172,8 @@ def qk_norm_rope(
         out = _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, offset, pos, float(eps),
                                   errors)
     else:
-        out = _forward(_rows(q), _rows(k), _native.contiguous16(q_weight), _native.contiguous16(k_weight), cos, sin, offset, pos,
-                       float(eps), errors)
+        weights = map(_native.contiguous16, (q_weight, k_weight))
+        out = _forward(_rows(q), _rows(k), *weights, cos, sin, offset, pos, float(eps), errors)
     if pos is not None and check:
         _raise_outside(errors, S, cos_cache.shape[0])
     return out
