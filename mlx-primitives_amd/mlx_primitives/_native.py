@@ -309,7 +309,7 @@ def require_no_grad(*tensors: Optional[torch.Tensor]) -> None:
 def require_no_tangent(*tensors: Optional[torch.Tensor]) -> None:
     """Refuse dual tensors of forward-mode differentiation, whose tangents the outputs
     would silently lack."""
-    if forward_ad._current_level < 0:
+    if getattr(forward_ad, "_current_level", 0) < 0:  # (nowhere within a dual_level)
         return
     if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("mlx_primitives (MI355X build) has no forward-mode derivatives; "

@@ -75,13 +75,18 @@ class BlockAllocator:
     Freed blocks are reused first (last in, first out), so a serving loop
     keeps touching the same pages. Thread-safe (re-entrant lock), as the
     reference (block_allocator.py:52-139).
+
+    clear_scales: 8-bit blocks are handed out with the scale 0, which writes of
+    single slots (set_block_data) need; a user that only appends, from slot 0 of
+    each block on, can do without.
     """
 
     def __init__(self, config: BlockConfig, num_blocks: int, enable_cow: bool = True,
-                 device=None) -> None:
+                 device=None, *, clear_scales: bool = True) -> None:
         self._config = config
         self._num_blocks = num_blocks
         self._enable_cow = enable_cow
+        self._clear_new = config.is_8bit and clear_scales
         self._lock = threading.RLock()
         self._device = torch.device(device) if device is not None else default_device()
         shape = (num_blocks,) + config.kv_shape
@@ -128,11 +133,11 @@ class BlockAllocator:
     def allocate(self, count: int = 1) -> List[int]:
         """Take `count` blocks (reference count 1 each); RuntimeError if the pool
         has fewer free blocks (block_allocator.py:142-167). Blocks of 8 bits start
-        with the scale 0 (a small device operation): what an earlier owner left in
-        them stands for nothing."""
+        with the scale 0, cleared on the current stream: what an earlier owner left
+        in them stands for nothing."""
         with self._lock:
             out = self._take(count)
-            if self._scales is not None and out:
+            if self._clear_new and out:
                 self._clear_scales(out)
             return out
 

@@ -113,7 +113,8 @@ class KVCache:
         self._page_tables: List[PageTable] = []
         for _ in range(config.num_layers):
             alloc = BlockAllocator(config.block_config, num_blocks=blocks,
-                                   enable_cow=config.enable_cow, device=device)
+                                   enable_cow=config.enable_cow, device=device,
+                                   clear_scales=False)  # (appends start each block anew)
             self._allocators.append(alloc)
             self._page_tables.append(PageTable(alloc))
         # user sequence id -> the sequence id in each layer's page table

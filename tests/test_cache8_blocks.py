@@ -50,6 +50,10 @@ def test_blocks_are_handed_out_empty(dtype):
     a.increment_ref(ids[0])
     new = a.copy_on_write(ids[0])
     assert new != ids[0] and all((s[new] == 3.0).all() for s in a.get_scales())
+    # who only appends does without
+    a = BlockAllocator(BlockConfig(16, 3, 32, dtype), 2, device="cpu", clear_scales=False)
+    a.get_scales()[0].fill_(7.0)
+    assert (a.get_scales()[0][a.allocate(2)] == 7.0).all()
 
 
 @pytest.mark.gpu
